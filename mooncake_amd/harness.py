@@ -19,6 +19,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _raw_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
+def _used_on(streams: Sequence[torch.cuda.Stream], *tensors: Optional[torch.Tensor]) -> None:
+    """Once these tensors are gone, their memory is given out again only behind what these streams have been given by then."""
+    for t in tensors:
+        if t is not None:
+            for stream in streams:
+                t.record_stream(stream)
+
+
 class WorldHarness:
     def __init__(self, cfg: EPConfig, device: str = "cuda", world: Optional[ep.World] = None,
                  num_tokens: Optional[Sequence[int]] = None):
@@ -223,13 +231,17 @@ class WorldHarness:
         c = self.cfg
         R, T = c.num_ranks, c.tokens_per_rank
         assert tuple(logits.shape) == (R, T, c.num_experts) and logits.is_contiguous()
-        if self.topk_idx is None:
-            self.topk_idx = torch.empty((R, T, c.num_topk), dtype=torch.int64, device=self.device)
-        if self.topk_weights is None:
-            self.topk_weights = torch.empty((R, T, c.num_topk), dtype=torch.float32, device=self.device)
+        caller = None if stream is None else torch.cuda.current_stream(self.device)
         with torch.cuda.stream(stream):
+            # (inside: memory taken back from another stream may still be in use there)
+            if self.topk_idx is None:
+                self.topk_idx = torch.empty((R, T, c.num_topk), dtype=torch.int64, device=self.device)
+            if self.topk_weights is None:
+                self.topk_weights = torch.empty((R, T, c.num_topk), dtype=torch.float32, device=self.device)
             operators.route(logits.view(R * T, -1), c.num_topk,
                             out=(self.topk_idx.view(R * T, -1), self.topk_weights.view(R * T, -1)), **kwargs)
+        if stream is not None:
+            _used_on((caller, stream), self.topk_idx, self.topk_weights)
 
     def experts(self, w_gate_up: operators.Scaled, w_down: operators.Scaled,
                 stream: Optional[torch.cuda.Stream] = None) -> None:
@@ -237,13 +249,16 @@ class WorldHarness:
         R * L of them: w_gate_up [R * L, 2I, H], w_down [R * L, H, I], the experts in their global order."""
         c = self.cfg
         E, RM, H = c.num_experts, c.num_ranks * c.max_tokens, c.hidden
-        if self.expert_out is None:
-            self.alloc_combine_io()
         x = self.recv_x_typed().view(E, RM, H)
         if c.use_fp8:
             x = (x, self.recv_scales_phys.view(E, H // 128, RM).transpose(1, 2))
+        caller = None if stream is None else torch.cuda.current_stream(self.device)
         with torch.cuda.stream(stream):
+            if self.expert_out is None:         # (inside, as in route)
+                self.alloc_combine_io()
             operators.expert_mlp(x, self.recv_count.view(E), w_gate_up, w_down, out=self.expert_out.view(E, RM, H))
+        if stream is not None:
+            _used_on((caller, stream), self.recv_x, self.recv_scales_phys, self.recv_count, self.expert_out, self.combined)
 
     def fill_expert_out_from_recv(self, factor_per_expert: Optional[torch.Tensor] = None) -> None:
         """Mock expert: expert_out = dequantised dispatched rows (times a per-expert
