@@ -39,6 +39,7 @@ class WorldHarness:
         self.x = self.topk_idx = self.topk_weights = None
         self.recv_x = self.recv_scales_phys = self.recv_count = self.src_info = self.layout_range = None
         self.expert_out = self.combined = None
+        self._routed = (None, None)     # what route writes to: tensors of the harness's own
         self.active_ranks = torch.ones((R, R), dtype=torch.int32, device=self.device)
         self._prepared = {}     # the latest marshalled whole-world calls, by everything that is marshalled (_key)
 
@@ -227,19 +228,19 @@ class WorldHarness:
 
     def route(self, logits: torch.Tensor, stream: Optional[torch.cuda.Stream] = None, **kwargs) -> None:
         """topk_idx, topk_weights = the router's choices for every rank's tokens (logits [R, T, E], contiguous), in one call;
-        kwargs: `mooncake_amd.route`'s."""
+        kwargs: `mooncake_amd.route`'s.  What `load` was given stays as it is."""
         c = self.cfg
         R, T = c.num_ranks, c.tokens_per_rank
         assert tuple(logits.shape) == (R, T, c.num_experts) and logits.is_contiguous()
         caller = None if stream is None else torch.cuda.current_stream(self.device)
         with torch.cuda.stream(stream):
-            # (inside: memory taken back from another stream may still be in use there)
-            if self.topk_idx is None:
-                self.topk_idx = torch.empty((R, T, c.num_topk), dtype=torch.int64, device=self.device)
-            if self.topk_weights is None:
-                self.topk_weights = torch.empty((R, T, c.num_topk), dtype=torch.float32, device=self.device)
-            operators.route(logits.view(R * T, -1), c.num_topk,
-                            out=(self.topk_idx.view(R * T, -1), self.topk_weights.view(R * T, -1)), **kwargs)
+            if self._routed[0] is None:
+                # (inside: memory taken back from another stream may still be in use there)
+                self._routed = (torch.empty((R, T, c.num_topk), dtype=torch.int64, device=self.device),
+                                torch.empty((R, T, c.num_topk), dtype=torch.float32, device=self.device))
+            idx, weights = self._routed
+            operators.route(logits.view(R * T, -1), c.num_topk, out=(idx.view(R * T, -1), weights.view(R * T, -1)), **kwargs)
+        self.topk_idx, self.topk_weights = idx, weights
         if stream is not None:
             _used_on((caller, stream), self.topk_idx, self.topk_weights)
 

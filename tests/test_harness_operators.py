@@ -83,3 +83,22 @@ def test_expert_rows_are_allocated_for_the_stream_that_writes_them(monkeypatch, 
     for t in (h.recv_x, h.recv_count) + ((h.recv_scales_phys,) if fp8 else ()):
         assert stream is None or "side" in seen.used_on[t.data_ptr()]
     assert seen.calls[0][1] == (stream or "caller")
+
+
+def test_what_was_loaded_is_not_written_over(monkeypatch):
+    Recorder(monkeypatch)
+    h = make()
+    data = {"x": torch.zeros(R, T, H, dtype=torch.bfloat16), "topk_idx": torch.full((R, T, K), 5),
+            "topk_weights": torch.full((R, T, K), 0.5)}
+    h.load(data)
+    h.route(torch.zeros(R, T, E))
+    assert bool((data["topk_idx"] == 5).all()) and bool((data["topk_weights"] == 0.5).all())
+    assert bool((h.topk_idx == 7).all()) and bool((h.topk_weights == 7).all())
+    # the next step's choices come to the same place, which a recorded dispatch reads; loaded ones come back by loading
+    at = h.topk_idx.data_ptr(), h.topk_weights.data_ptr()
+    h.route(torch.zeros(R, T, E))
+    assert at == (h.topk_idx.data_ptr(), h.topk_weights.data_ptr())
+    h.load(data)
+    assert bool((h.topk_idx == 5).all())
+    h.route(torch.zeros(R, T, E))
+    assert bool((data["topk_idx"] == 5).all()) and at == (h.topk_idx.data_ptr(), h.topk_weights.data_ptr())
