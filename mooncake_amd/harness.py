@@ -8,7 +8,7 @@ Per-rank tensors are slices of rank-major allocations, so rank r's
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -25,6 +25,15 @@ def _used_on(streams: Sequence[torch.cuda.Stream], *tensors: Optional[torch.Tens
         if t is not None:
             for stream in streams:
                 t.record_stream(stream)
+
+
+def _runs(present: Optional[Sequence[int]], R: int) -> List[Tuple[int, int]]:
+    """The ranks that are present, as [first, last) of each run of them."""
+    here = [True] * R if present is None else [bool(p) for p in present]
+    assert len(here) == R
+    begins = [r for r in range(R) if here[r] and (r == 0 or not here[r - 1])]
+    ends = [r + 1 for r in range(R) if here[r] and (r + 1 == R or not here[r + 1])]
+    return list(zip(begins, ends))
 
 
 class WorldHarness:
@@ -245,19 +254,23 @@ class WorldHarness:
             _used_on((caller, stream), self.topk_idx, self.topk_weights)
 
     def experts(self, w_gate_up: operators.Scaled, w_down: operators.Scaled,
-                stream: Optional[torch.cuda.Stream] = None) -> None:
+                stream: Optional[torch.cuda.Stream] = None, present: Optional[Sequence[int]] = None) -> None:
         """expert_out = every rank's experts over the rows dispatch left (`mooncake_amd.expert_mlp`), in one call over all
-        R * L of them: w_gate_up [R * L, 2I, H], w_down [R * L, H, I], the experts in their global order."""
+        R * L of them: w_gate_up [R * L, 2I, H], w_down [R * L, H, I], the experts in their global order.  present[r] == 0
+        leaves out rank r, whose recv_count is not dispatch's then (a call for each run of present ranks)."""
         c = self.cfg
-        E, RM, H = c.num_experts, c.num_ranks * c.max_tokens, c.hidden
-        x = self.recv_x_typed().view(E, RM, H)
-        if c.use_fp8:
-            x = (x, self.recv_scales_phys.view(E, H // 128, RM).transpose(1, 2))
+        R, L, E, RM, H = c.num_ranks, c.num_local_experts, c.num_experts, c.num_ranks * c.max_tokens, c.hidden
         caller = None if stream is None else torch.cuda.current_stream(self.device)
         with torch.cuda.stream(stream):
             if self.expert_out is None:         # (inside, as in route)
                 self.alloc_combine_io()
-            operators.expert_mlp(x, self.recv_count.view(E), w_gate_up, w_down, out=self.expert_out.view(E, RM, H))
+            x, count, out = self.recv_x_typed().view(E, RM, H), self.recv_count.view(E), self.expert_out.view(E, RM, H)
+            if c.use_fp8:
+                x = (x, self.recv_scales_phys.view(E, H // 128, RM).transpose(1, 2))
+            for first, last in _runs(present, R):
+                def cut(v, of=slice(first * L, last * L)):
+                    return tuple(t[of] for t in v) if isinstance(v, (tuple, list)) else v[of]
+                operators.expert_mlp(cut(x), cut(count), cut(w_gate_up), cut(w_down), out=cut(out))
         if stream is not None:
             _used_on((caller, stream), self.recv_x, self.recv_scales_phys, self.recv_count, self.expert_out, self.combined)
 

@@ -102,3 +102,24 @@ def test_what_was_loaded_is_not_written_over(monkeypatch):
     assert bool((h.topk_idx == 5).all())
     h.route(torch.zeros(R, T, E))
     assert bool((data["topk_idx"] == 5).all()) and at == (h.topk_idx.data_ptr(), h.topk_weights.data_ptr())
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("present,runs", [(None, [(0, 3)]), ((1, 1, 1), [(0, 3)]), ((1, 0, 1), [(0, 1), (2, 3)]),
+                                          ((0, 1, 1), [(1, 3)]), ((0, 0, 0), [])])
+def test_experts_of_silent_ranks_are_left_out(monkeypatch, present, runs, fp8):
+    seen = Recorder(monkeypatch)
+    h = make(fp8)
+    w_gate_up, w_down = torch.zeros(E, 2 * I, H), torch.zeros(E, H, I)
+    if fp8:
+        w_gate_up, w_down = (w_gate_up, torch.zeros(E, 2 * I // 128, H // 128)), (w_down, torch.zeros(E, H // 128, I // 128))
+    h.experts(w_gate_up, w_down, **({} if present is None else {"present": present}))
+    L = E // R
+    assert len(seen.calls) == len(runs)
+    for (first, last), (_, _, x, count, w1, w2, out) in zip(runs, seen.calls):
+        x, w1, w2 = (v if fp8 else (v,) for v in (x, w1, w2))
+        for got, of in ([(x[0], h.recv_x.view(E, R * T, H)), (count, h.recv_count.view(E)), (out, h.expert_out.view(E, R * T, H))]
+                        + list(zip(w1, w_gate_up if fp8 else (w_gate_up,))) + list(zip(w2, w_down if fp8 else (w_down,)))
+                        + ([(x[1], h.recv_scales_phys.view(E, -1, R * T).transpose(1, 2))] if fp8 else [])):
+            part = of[first * L:last * L]
+            assert got.shape == part.shape and got.data_ptr() == part.data_ptr() and got.stride() == part.stride()
