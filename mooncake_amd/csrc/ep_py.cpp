@@ -612,22 +612,6 @@ py::tuple route_tensors(py::object logits_, int num_topk, bool sigmoid, py::obje
         need_tensor(*mask, at::kBool, device);
         MC_CHECK(mask->dim() == 1 && mask->size(0) == T);
     }
-    if (idx_.is_none() && weights_.is_none()) {
-        // one allocation for both (a second one is 0.7 us of a call of few tokens' 5), the indices first and the weights at the
-        // alignment that they would have alone
-        const int64_t places = T * num_topk, behind = (places * 2 + 127) / 128 * 128;
-        const c10::Storage both = empty({behind + places}, at::kFloat, logits.device()).storage();
-        const auto part = [&](at::ScalarType type, int64_t offset) {
-            at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-                c10::Storage(both), c10::DispatchKeySet(c10::computeDispatchKey(type, c10::nullopt, logits.device())),
-                c10::scalarTypeToTypeMeta(type));
-            t.unsafeGetTensorImpl()->set_sizes_contiguous({T, num_topk});
-            t.unsafeGetTensorImpl()->set_storage_offset(offset);
-            return wrap_tensor(std::move(t));
-        };
-        idx_ = part(at::kLong, 0);
-        weights_ = part(at::kFloat, behind);
-    }
     if (idx_.is_none()) idx_ = wrap_tensor(empty({T, num_topk}, at::kLong, logits.device()));
     if (weights_.is_none()) weights_ = wrap_tensor(empty({T, num_topk}, at::kFloat, logits.device()));
     const at::Tensor &idx = tensor_of(idx_), &weights = tensor_of(weights_);
