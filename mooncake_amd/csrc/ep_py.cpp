@@ -653,8 +653,10 @@ py::tuple expert_gate_up_tensors(py::object x_, py::object scales_, py::object c
     need_tensor(count, at::kInt, device);
     MC_CHECK(count.dim() == 1 && count.size(0) == L);
     if (fp8) need_scales(*scales, L, rows, H / 128, device);
-    if (act_.is_none()) act_ = wrap_tensor(empty({L, rows, I}, x.scalar_type(), x.device()));
-    if (fp8 && act_scales_.is_none()) act_scales_ = wrap_tensor(empty({L, I / 128, rows}, at::kFloat, x.device()).transpose(1, 2));
+    if (act_.is_none()) {       // (values handed in without their scales are refused below)
+        act_ = wrap_tensor(empty({L, rows, I}, x.scalar_type(), x.device()));
+        if (fp8) act_scales_ = wrap_tensor(empty({L, I / 128, rows}, at::kFloat, x.device()).transpose(1, 2));
+    }
     const at::Tensor& act = tensor_of(act_);
     need_tensor(act, x.scalar_type(), device);
     MC_CHECK(act.dim() == 3 && act.size(0) == L && act.size(1) == rows && act.size(2) == I);
