@@ -276,7 +276,8 @@ int mc_ep_route(uint64_t logits_ptr, int logits_bf16, int64_t logits_row_stride,
  * multiple of 128 (up to 32768 with use_fp8); intermediate of 128 (up to
  * 32768) with use_fp8, else of 8; L <= 2048; rows_per_expert <= 2^24; x, w, act
  * and out are 16-byte aligned; one expert's weights of a call take less than
- * 2 GiB.  Counts beyond 0 .. rows_per_expert are taken as the nearer of the two.
+ * 2 GiB; input and output rows (and their scales) lie apart.  Counts beyond
+ * 0 .. rows_per_expert are taken as the nearer of the two.
  * Both enqueue one kernel on stream_ptr, allocate nothing and may be recorded
  * into a graph. */
 int mc_ep_expert_gate_up(uint64_t packed_recv_x_ptr, uint64_t packed_recv_x_scales_ptr,

@@ -591,6 +591,11 @@ int launch(const ExpertArgs& a, bool fp8, hipStream_t stream) {
 constexpr int64_t kMostBytes = (int64_t)1 << 31;   // of one expert's weights and a tile past them: offsets within are 32 bits
 constexpr int kMostRows = 1 << 24;                 // of an expert: up to there the plan's divisions by multiplication are exact
 
+// Other blocks still read what one writes over: input and output have to lie apart.
+bool apart(uint64_t a, int64_t a_bytes, uint64_t b, int64_t b_bytes) {
+    return a + (uint64_t)a_bytes <= b || b + (uint64_t)b_bytes <= a;
+}
+
 }  // namespace
 }  // namespace mcep
 
@@ -614,6 +619,10 @@ int mc_ep_expert_gate_up(uint64_t packed_recv_x_ptr, uint64_t packed_recv_x_scal
     OP_ASSERT((2 * (int64_t)intermediate + 256) * row < kMostBytes);
     OP_ASSERT(!use_fp8 || hidden <= kMaxGroups * 128);
     OP_ASSERT((int64_t)num_local_experts * (rows_per_expert / 32 + 1) * (intermediate / 64 + 1) < kMostBytes);
+    const int64_t rows = (int64_t)num_local_experts * rows_per_expert;
+    OP_ASSERT(apart(packed_recv_x_ptr, rows * row, act_ptr, rows * intermediate * (use_fp8 ? 1 : 2)));
+    OP_ASSERT(!use_fp8 || apart(packed_recv_x_scales_ptr, rows * (hidden / 128) * 4, act_scales_ptr,
+                                rows * (intermediate / 128) * 4));
     ExpertArgs a{(const char*)packed_recv_x_ptr, (const float*)packed_recv_x_scales_ptr, (const int32_t*)packed_recv_count_ptr,
                  (const char*)w_ptr, (const float*)w_scales_ptr, (char*)act_ptr, (float*)act_scales_ptr, num_local_experts,
                  rows_per_expert, intermediate, (int)row};
@@ -635,6 +644,8 @@ int mc_ep_expert_down(uint64_t act_ptr, uint64_t act_scales_ptr, uint64_t packed
     OP_ASSERT(((int64_t)hidden + 256) * row < kMostBytes);
     OP_ASSERT(!use_fp8 || intermediate <= kMaxGroups * 128);
     OP_ASSERT((int64_t)num_local_experts * (rows_per_expert / 32 + 1) * (hidden / 128 + 1) < kMostBytes);
+    const int64_t rows = (int64_t)num_local_experts * rows_per_expert;
+    OP_ASSERT(apart(act_ptr, rows * row, out_ptr, rows * hidden * 2));
     ExpertArgs a{(const char*)act_ptr, (const float*)act_scales_ptr, (const int32_t*)packed_recv_count_ptr,
                  (const char*)w_ptr, (const float*)w_scales_ptr, (char*)out_ptr, nullptr, num_local_experts,
                  rows_per_expert, hidden, (int)row};

@@ -102,7 +102,7 @@ def expert_gate_up(packed_recv_x: Scaled, packed_recv_count: torch.Tensor, w_gat
     column-major per expert).  w_gate_up: [L, 2I, H], Wg's rows first - bf16, or (fp8 values, f32 scales of their 128 x 128
     blocks [L, 2I/128, H/128]) for an fp8 payload.  Returns (or writes to `act`) bf16 [L, R*max, I], or (fp8 values, f32
     scales [L, R*max, I/128]) laid out like the payload, a scale being amax / 448 with amax at least 1e-4.  I is a multiple
-    of 128 in fp8, of 8 in bf16."""
+    of 128 in fp8, of 8 in bf16.  `act` may not lie on the payload."""
     x, scales = _parts(packed_recv_x)
     w, w_scales = _parts(w_gate_up)
     a, a_scales = (None, None) if act is None else _parts(act)
@@ -129,7 +129,7 @@ def expert_down(act: Scaled, packed_recv_count: torch.Tensor, w_down: Scaled,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[e] = act[e] Wd[e]^T, bf16 [L, R*max, H], for the first packed_recv_count[e] rows of every local expert: what
     combine reads.  act as `expert_gate_up` returns it; w_down [L, H, I], bf16 or (fp8 values, f32 scales of their
-    128 x 128 blocks [L, H/128, I/128])."""
+    128 x 128 blocks [L, H/128, I/128]).  `out` may not lie on the activations."""
     a, a_scales = _parts(act)
     w, w_scales = _parts(w_down)
     device, stream = _here()
