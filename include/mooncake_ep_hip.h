@@ -242,7 +242,7 @@ int mc_ep_world_combine_packed(mc_ep_world_t* world, const uint64_t* packed_recv
  * (f32, or bf16 when logits_bf16; rows logits_row_stride elements apart) ->
  * topk_idx int64 and topk_weights f32 [num_tokens, num_topk], as dispatch and
  * combine take them.  scores = softmax over the experts, or sigmoid when
- * sigmoid_scores, in 32 bits.  The choice goes by scores + bias (bias_ptr: f32
+ * sigmoid_scores, in 32 bits (a sigmoid is zero for logits below -88.72).  The choice goes by scores + bias (bias_ptr: f32
  * [num_experts]) or, without a bias (0), by the logits; with num_groups > 1
  * only inside the num_topk_groups groups of consecutive experts whose largest
  * choice - with a bias: whose two largest together - is best.  Equal values

@@ -60,14 +60,34 @@ __device__ __forceinline__ float taken_logit(float v) {
     return fminf(v, FLT_MAX);
 }
 
-// The same value as 1 / (1 + exp(-x)) on a tensor has, to the last bit, which decides between nearly equal scores.  The
-// quotient: the hardware's reciprocal and one Newton step are the correctly rounded 1 / d for every d from 1 to 2^126
-// (all mantissas tried); beyond that the score is less than the smallest normal number and counts as zero.
+// Scores of logits as taken_logit gives them: the same values as 1 / (1 + exp(-x)) on a tensor has, to the last bit, which
+// decides between nearly equal scores.  The quotient: the hardware's reciprocal and one Newton step are the correctly
+// rounded 1 / d for every d from 1 to 2^126 (all mantissas tried); beyond that the score is less than the smallest normal
+// number, which the reciprocal does not give, and is divided out (zero from the overflow of the exponential on, for logits
+// below -88.72).  One branch for all of a lane's, the biases asked for in front of it: 131072 tokens of 256 experts 84 us
+// and of 384 113, as without it (83, 111); with the biases behind it 88 and 122, with a branch for each 90 and 129.
+template <int N>
+__device__ __forceinline__ void sigmoids(const float (&x)[N], float (&s)[N]) {
+    bool small = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float d = 1.0f + expf(-x[j]);
+        const float r = __builtin_amdgcn_rcpf(d);
+        const float q = fmaf(fmaf(-d, r, 1.0f), r, r);
+        s[j] = d < 0x1p126f ? q : 0.0f;
+        small |= !(d < 0x1p126f) & (x[j] > -INFINITY);
+    }
+    if (__builtin_expect(small, 0)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (s[j] == 0.0f) s[j] = 1.0f / (1.0f + expf(-x[j]));
+    }
+}
 __device__ __forceinline__ float sigmoid(float x) {
-    const float d = 1.0f + expf(-x);
-    const float r = __builtin_amdgcn_rcpf(d);
-    const float q = fmaf(fmaf(-d, r, 1.0f), r, r);
-    return d < 0x1p126f ? q : 0.0f;
+    const float of[1] = {x};
+    float s[1];
+    sigmoids(of, s);
+    return s[0];
 }
 
 // floats in their order as integers (both zeros the same one), and back
@@ -191,10 +211,18 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void route_wave_kernel(RouteAr
         for (int j = 0; j < NV; ++j) c[j] = ordered(x[j]);
     }
     if (a.bias != nullptr) {
+        float s[NV], b[NV];       // (on their way while the scores are computed: see sigmoids)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) b[j] = a.bias[lane * NV + j < a.E ? lane * NV + j : 0];
+        if (SOFTMAX) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) s[j] = expf(x[j] - top) / total;
+        } else {
+            sigmoids(x, s);
+        }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = lane * NV + j;
-            const float v = (SOFTMAX ? expf(x[j] - top) / total : sigmoid(x[j])) + a.bias[e < a.E ? e : 0];
+            const float v = s[j] + b[j];
             c[j] = x[j] > -INFINITY && v > -INFINITY ? ordered(v) : kNever;
         }
     }
@@ -363,9 +391,11 @@ __global__ __launch_bounds__(64) void route_thread_kernel(RouteArgs a) {
     }
     if (top == -INFINITY) top = 0.0f;
     float s[N];
+    if (SOFTMAX) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        s[j] = SOFTMAX ? expf(x[j] - top) : sigmoid(x[j]);
+        for (int j = 0; j < N; ++j) s[j] = expf(x[j] - top);
+    } else {
+        sigmoids(x, s);
     }
     if (SOFTMAX) {      // in pairs of pairs, as the lanes of a wave add
         float part[N];

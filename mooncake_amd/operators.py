@@ -53,7 +53,8 @@ def route(logits: torch.Tensor, num_topk: int, score: str = "softmax", bias: Opt
     """Router logits [T, E] (f32 or bf16, any row stride) -> (topk_idx int64, topk_weights f32), both [T, num_topk]:
     what `Buffer.dispatch` and `Buffer.combine` take.
 
-    The scores are softmax (over the experts) or sigmoid of the logits, in 32 bits.  Experts are chosen by score + bias
+    The scores are softmax (over the experts) or sigmoid of the logits, in 32 bits (a sigmoid is zero for logits below
+    -88.72).  Experts are chosen by score + bias
     (bias f32 [E]) or, without one, by their logits - the same order -, in falling order, the lowest index first among
     equals.  With num_groups > 1 the experts are that many equal groups of consecutive ones and only those of the best
     topk_groups groups can be chosen; a group counts as its best expert, with a bias as its best two together.  The
