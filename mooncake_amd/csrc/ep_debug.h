@@ -50,6 +50,14 @@ int mc_ep_debug_gather_rows(uint64_t dst_ptr, uint64_t src_ptr, int row_bytes, i
 int mc_ep_debug_scatter_rows(uint64_t dst_ptr, uint64_t src_ptr, int row_bytes, int64_t in_rows, int regions,
                              int64_t region_rows, int used, uint64_t stream_ptr);
 
+/* How an expert's product of these counts (in host memory) is cut: the rows of a tile at most, its weight rows (256 or
+ * 128), the tiles of rows of all experts together, and whether the weights are read past the caches.  columns and
+ * row_bytes: the output's columns and the bytes of a row of its input; blocks: that the kernel is launched with.  Tests
+ * ask which tiles a call runs: the kernel decides it by the same prices. */
+int mc_ep_debug_expert_plan(const int32_t* counts, int num_local_experts, int rows_per_expert, int columns, int row_bytes,
+                            int use_fp8, int gate_up, int blocks, int32_t* tile_rows, int32_t* weight_rows,
+                            int32_t* tiles, int32_t* streamed_weights);
+
 #ifdef __cplusplus
 }
 #endif

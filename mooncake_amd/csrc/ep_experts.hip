@@ -38,6 +38,8 @@
 #include <string>
 #include <type_traits>
 
+#include "ep_debug.h"
+#include "ep_expert_plan.h"
 #include "ep_operators.h"
 
 namespace mcep {
@@ -54,7 +56,6 @@ constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * 64;
 constexpr int kMaxLocalExperts = 2048;
 constexpr int kXCDs = 8;
-constexpr int kStep = 128;             // bytes of a row per K step
 constexpr int kMaxGroups = 256;        // scale groups of a row: fp8 rows of at most 32768
 
 struct ExpertArgs {
@@ -149,7 +150,7 @@ __device__ __forceinline__ Tile run_tiles(const ExpertArgs& a, Tile tile, const 
     const int wm = wave / C::WN, wn = wave % C::WN;
     const int quarter = lane >> 4, l16 = lane & 15;
     const int Kb = a.Kb;
-    const int steps = (Kb + kStep - 1) / kStep;
+    const int steps = steps_of(Kb);
     const int groups = Kb / kStep;                 // scale groups of a row (fp8: Kb is whole steps)
 
     // --- addresses of the loads: row of the tile = load * 64 + wave * 8 + lane / 8, 16-byte chunk (lane & 7) ^ (row & 7)
@@ -437,20 +438,6 @@ __device__ __forceinline__ Tile run_tiles(const ExpertArgs& a, Tile tile, const 
     }
 }
 
-// The plans a block can choose from: an expert's rows spread over as few tiles as give none more than 32 * blocks rows,
-// tiles of 256 or (the last four; not for fp8 gate_up, whose scale groups want 256) 128 weight rows.
-constexpr int kPlans = 12, kWidePlans = 8;
-// What a K step of a tile costs, in ns, by its blocks of 32 rows, and a tile besides (fitted to calls of every plan; the plan
-// that comes out is within 3 % of the best of the twelve for 4 to 256 experts of 24 to 512 rows, where the best is anything
-// from 32 x 256 and 64 x 128 to 256 x 256 and the worst takes 1.5 to 4 times as long).
-__device__ __forceinline__ int step_cost(bool wide, int blocks) { return wide ? 350 + 150 * blocks : 250 + 90 * blocks; }
-constexpr int kTileCost = 4000;
-// Few rows (all experts' are one tile each, and at most 32): the weights are read once and are the whole cost.  Where a
-// call reads more of them than the last-level cache is likely to keep until the next, they are read without a place in
-// the caches (8 experts of 44 MB fp8: 58 + 27 us kept, 53 + 24 not); fewer may be there from the call before (9 of
-// 2.2 MB: 10.7 + 7.4 us kept, 12.5 + 8.1 not).
-constexpr int64_t kStreamed = 64 << 20;
-
 template <bool FP8, bool GATE_UP>
 __global__ __launch_bounds__(kThreads, 2) void expert_kernel(ExpertArgs a) {
     __shared__ __align__(1024) char smem[kLdsBytes];
@@ -462,47 +449,42 @@ __global__ __launch_bounds__(kThreads, 2) void expert_kernel(ExpertArgs a) {
     // later).  Code that runs once is fetched for it: this is written to be short.
     int* sums = (int*)smem;                         // tiles and cost by plan
     if (threadIdx.x < 32) sums[threadIdx.x] = 0;
-    const int choice = lane & 15, blocks_most = choice < kWidePlans ? choice + 1 : choice + 1 - kWidePlans;
-    const bool wide = choice < kWidePlans;
-    const uint32_t per_most = 0xffffffffu / (uint32_t)(32 * blocks_most) + 1;     // x * this >> 32 is x / most, for the x there are
+    const int choice = lane & 15, choice_most = 32 * plan_blocks(choice);
+    const bool wide = plan_wide(choice);
+    const uint32_t per_most = divisor(choice_most);
     int tiles_sum = 0, cost_sum = 0;
     __syncthreads();
     for (int e = wave * 4 + (lane >> 4); e < a.L; e += 4 * kWaves) {
         int n = a.count[e];
         n = n < 0 ? 0 : (n > a.RM ? a.RM : n);
-        const int down = (int)__umulhi((uint32_t)(n + 32 * blocks_most - 1), per_most);
+        const int down = row_tiles(n, choice_most, per_most);
         tiles_sum += down;
-        if (n > 0) cost_sum += down * step_cost(wide, (int)ceilf((float)n * __builtin_amdgcn_rcpf((float)down) * 0.03125f));
+        cost_sum += rows_cost(n, down, wide);
     }
     atomicAdd(&sums[choice * 2], tiles_sum);
     atomicAdd(&sums[choice * 2 + 1], cost_sum);
     __syncthreads();
     int plan;
     {
-        const int steps = (a.Kb + kStep - 1) / kStep;
-        const int tiles = sums[choice * 2], cost = sums[choice * 2 + 1];
-        const int columns = (wide ? 256 : 128) / (GATE_UP ? 2 : 1);
-        const float across = (float)((a.N + columns - 1) / columns);
-        // rounds of the CUs, each as long as a tile of middling cost
-        const float rounds = ceilf((float)tiles * across / (float)gridDim.x);
-        float time = rounds * ((float)cost * __builtin_amdgcn_rcpf((float)(tiles > 0 ? tiles : 1)) * steps + kTileCost);
+        const int columns = plan_columns(choice, GATE_UP);
+        float time = plan_time(sums[choice * 2], sums[choice * 2 + 1], (a.N + columns - 1) / columns, gridDim.x, steps_of(a.Kb));
         if (choice >= (FP8 && GATE_UP ? kWidePlans : kPlans)) time = INFINITY;
         float least = time;
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) least = fminf(least, __shfl_xor(least, d));
         plan = __builtin_ctz((uint32_t)__ballot(time == least) & 0xffff);
     }
-    const int most = 32 * (plan < kWidePlans ? plan + 1 : plan + 1 - kWidePlans), bn = plan < kWidePlans ? 256 : 128;
+    const int most = 32 * plan_blocks(plan), bn = plan_wide(plan) ? 256 : 128;
     // --- begin[e], by every wave for itself (the same values)
     int experts;               // that have rows
     {
-        const uint32_t per = 0xffffffffu / (uint32_t)most + 1;
+        const uint32_t per = divisor(most);
         int total = 0;
         experts = 0;
         for (int e0 = 0; e0 < a.L; e0 += 64) {
             int n = e0 + lane < a.L ? a.count[e0 + lane] : 0;
             n = n < 0 ? 0 : (n > a.RM ? a.RM : n);
-            int sum = (int)__umulhi((uint32_t)(n + most - 1), per);
+            int sum = row_tiles(n, most, per);
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const int v = __shfl_up(sum, d);
@@ -516,10 +498,10 @@ __global__ __launch_bounds__(kThreads, 2) void expert_kernel(ExpertArgs a) {
     }
     __syncthreads();           // (the sums have been read: the stages are there now)
 
-    const int columns = GATE_UP ? bn / 2 : bn;
+    const int columns = plan_columns(plan, GATE_UP);
     const uint32_t across = (uint32_t)((a.N + columns - 1) / columns);
     const uint64_t tiles = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(begin[a.L]) * across;      // (less than 2^31: checked)
-    const bool once = __builtin_amdgcn_readfirstlane(begin[a.L]) == experts && (int64_t)tiles * bn * a.Kb >= kStreamed;
+    const bool once = streamed(__builtin_amdgcn_readfirstlane(begin[a.L]), experts, (int)across, bn, a.Kb);
     const uint32_t xcd = blockIdx.x % kXCDs, slots = gridDim.x / kXCDs;
     const uint32_t end = (uint32_t)(tiles * (xcd + 1) / kXCDs);
     uint32_t t = (uint32_t)(tiles * xcd / kXCDs) + blockIdx.x / kXCDs;
@@ -650,6 +632,34 @@ int mc_ep_expert_down(uint64_t act_ptr, uint64_t act_scales_ptr, uint64_t packed
                  (const char*)w_ptr, (const float*)w_scales_ptr, (char*)out_ptr, nullptr, num_local_experts,
                  rows_per_expert, hidden, (int)row};
     return launch<false>(a, use_fp8 != 0, (hipStream_t)stream_ptr);
+}
+
+int mc_ep_debug_expert_plan(const int32_t* counts, int num_local_experts, int rows_per_expert, int columns, int row_bytes,
+                            int use_fp8, int gate_up, int blocks, int32_t* tile_rows, int32_t* weight_rows, int32_t* tiles,
+                            int32_t* streamed_weights) {
+    OP_ASSERT(num_local_experts >= 0 && num_local_experts <= kMaxLocalExperts);
+    OP_ASSERT(rows_per_expert >= 0 && rows_per_expert <= kMostRows);
+    OP_ASSERT(columns > 0 && row_bytes > 0 && blocks > 0);
+    float least = INFINITY;
+    for (int plan = 0; plan < (use_fp8 && gate_up ? kWidePlans : kPlans); ++plan) {
+        const int most = 32 * plan_blocks(plan), across = (columns - 1) / plan_columns(plan, gate_up) + 1;
+        int sum = 0, cost = 0, experts = 0;
+        for (int e = 0; e < num_local_experts; ++e) {
+            const int n = counts[e] < 0 ? 0 : counts[e] > rows_per_expert ? rows_per_expert : counts[e];
+            const int down = row_tiles(n, most, divisor(most));
+            sum += down;
+            cost += rows_cost(n, down, plan_wide(plan));
+            experts += n > 0;
+        }
+        const float time = plan_time(sum, cost, across, blocks, steps_of(row_bytes));
+        if (!(time < least)) continue;
+        least = time;
+        *tile_rows = most;
+        *weight_rows = plan_wide(plan) ? 256 : 128;
+        *tiles = sum;
+        *streamed_weights = plan == 0 && streamed(sum, experts, across, 256, row_bytes);
+    }
+    return MC_EP_OK;
 }
 
 }  // extern "C"
