@@ -45,9 +45,9 @@ __host__ __device__ __forceinline__ int rows_cost(int n, int down, bool wide) {
     return n > 0 ? down * step_cost(wide, (int)ceilf((float)n * price_reciprocal((float)down) * 0.03125f)) : 0;
 }
 
-// A call of `tiles` tiles of rows, whose K steps cost `cost` together, by `across` tiles of columns on `blocks` blocks: rounds
-// of the blocks, each as long as a tile of middling cost.
-__host__ __device__ __forceinline__ float plan_time(int tiles, int cost, int across, int blocks, int steps) {
+// A call of `tiles` tiles of rows, whose K steps cost `cost` together (past 31 bits from 1.4 million tiles on), by `across`
+// tiles of columns on `blocks` blocks: rounds of the blocks, each as long as a tile of middling cost.
+__host__ __device__ __forceinline__ float plan_time(int tiles, uint64_t cost, int across, int blocks, int steps) {
     const float rounds = ceilf((float)tiles * (float)across / (float)blocks);
     return rounds * ((float)cost * price_reciprocal((float)(tiles > 0 ? tiles : 1)) * steps + kTileCost);
 }

@@ -447,12 +447,17 @@ __global__ __launch_bounds__(kThreads, 2) void expert_kernel(ExpertArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // --- the plan.  A lane in sixteen tries a plan, on every 32nd expert; its sums meet in LDS (behind which the stages begin
     // later).  Code that runs once is fetched for it: this is written to be short.
-    int* sums = (int*)smem;                         // tiles and cost by plan
-    if (threadIdx.x < 32) sums[threadIdx.x] = 0;
+    unsigned long long* cost_sums = (unsigned long long*)smem;      // cost and tiles by plan
+    int* tile_sums = (int*)(cost_sums + 16);
+    if (threadIdx.x < 16) {
+        cost_sums[threadIdx.x] = 0;
+        tile_sums[threadIdx.x] = 0;
+    }
     const int choice = lane & 15, choice_most = 32 * plan_blocks(choice);
     const bool wide = plan_wide(choice);
     const uint32_t per_most = divisor(choice_most);
-    int tiles_sum = 0, cost_sum = 0;
+    int tiles_sum = 0;
+    unsigned long long cost_sum = 0;
     __syncthreads();
     for (int e = wave * 4 + (lane >> 4); e < a.L; e += 4 * kWaves) {
         int n = a.count[e];
@@ -461,13 +466,13 @@ __global__ __launch_bounds__(kThreads, 2) void expert_kernel(ExpertArgs a) {
         tiles_sum += down;
         cost_sum += rows_cost(n, down, wide);
     }
-    atomicAdd(&sums[choice * 2], tiles_sum);
-    atomicAdd(&sums[choice * 2 + 1], cost_sum);
+    atomicAdd(&tile_sums[choice], tiles_sum);
+    atomicAdd(&cost_sums[choice], cost_sum);
     __syncthreads();
     int plan;
     {
         const int columns = plan_columns(choice, GATE_UP);
-        float time = plan_time(sums[choice * 2], sums[choice * 2 + 1], (a.N + columns - 1) / columns, gridDim.x, steps_of(a.Kb));
+        float time = plan_time(tile_sums[choice], cost_sums[choice], (a.N + columns - 1) / columns, gridDim.x, steps_of(a.Kb));
         if (choice >= (FP8 && GATE_UP ? kWidePlans : kPlans)) time = INFINITY;
         float least = time;
 #pragma unroll
@@ -643,7 +648,8 @@ int mc_ep_debug_expert_plan(const int32_t* counts, int num_local_experts, int ro
     float least = INFINITY;
     for (int plan = 0; plan < (use_fp8 && gate_up ? kWidePlans : kPlans); ++plan) {
         const int most = 32 * plan_blocks(plan), across = (columns - 1) / plan_columns(plan, gate_up) + 1;
-        int sum = 0, cost = 0, experts = 0;
+        int sum = 0, experts = 0;
+        uint64_t cost = 0;
         for (int e = 0; e < num_local_experts; ++e) {
             const int n = counts[e] < 0 ? 0 : counts[e] > rows_per_expert ? rows_per_expert : counts[e];
             const int down = row_tiles(n, most, divisor(most));
