@@ -239,10 +239,11 @@ int mc_ep_world_combine_packed(mc_ep_world_t* world, const uint64_t* packed_recv
 /* ---- the router and the experts ------------------------------------------ */
 
 /* What stands in front of dispatch: router logits [num_tokens, num_experts]
- * (f32, or bf16 when logits_bf16; rows logits_row_stride elements apart) ->
- * topk_idx int64 and topk_weights f32 [num_tokens, num_topk], as dispatch and
- * combine take them.  scores = softmax over the experts, or sigmoid when
- * sigmoid_scores, in 32 bits (a sigmoid is zero for logits below -88.72).  The choice goes by scores + bias (bias_ptr: f32
+ * (f32, or bf16 when logits_bf16; rows logits_row_stride elements apart, at
+ * least num_experts) -> topk_idx int64 and topk_weights f32 [num_tokens,
+ * num_topk], as dispatch and combine take them.  scores = softmax over the
+ * experts, or sigmoid when sigmoid_scores, in 32 bits (a sigmoid is zero for
+ * logits below -88.72).  The choice goes by scores + bias (bias_ptr: f32
  * [num_experts]) or, without a bias (0), by the logits; with num_groups > 1
  * only inside the num_topk_groups groups of consecutive experts whose largest
  * choice - with a bias: whose two largest together - is best.  Equal values
@@ -271,13 +272,17 @@ int mc_ep_route(uint64_t logits_ptr, int logits_bf16, int64_t logits_row_stride,
  * weights are fp8 e4m3 with a f32 scale per 128 x 128 block ([L, rows / 128,
  * columns / 128]), and act is fp8 with a scale per 128 elements, amax / 448
  * with amax at least 1e-4, laid out like the payload's
- * ([L, intermediate / 128, rows_per_expert]).  Products are summed in 32 bits.
- * A stack of all ranks' tensors is one call with L = num_experts.  hidden is a
- * multiple of 128 (up to 32768 with use_fp8); intermediate of 128 (up to
- * 32768) with use_fp8, else of 8; L <= 2048; rows_per_expert <= 2^24; x, w, act
- * and out are 16-byte aligned; one expert's weights of a call take less than
- * 2 GiB; input and output rows (and their scales) lie apart.  Counts beyond
- * 0 .. rows_per_expert are taken as the nearer of the two.
+ * ([L, intermediate / 128, rows_per_expert]).  bf16 products are summed in 32
+ * bits.  fp8 products of eight consecutive elements are each cut off 2^-13 below
+ * the largest of the eight (the matrix instruction's own sum); from eight to
+ * eight, and between the groups of 128, sums have 32 bits.  act is rounded to
+ * its type between the two products.  A stack of all ranks' tensors is one call
+ * with L = num_experts.  hidden is a multiple of 128 (up to 32768 with use_fp8);
+ * intermediate of 128 (up to 32768) with use_fp8, else of 8; L <= 2048;
+ * rows_per_expert <= 2^24; x, w, act and out are 16-byte aligned; one expert's
+ * weights of a call take less than 2 GiB; input and output rows (and their
+ * scales) lie apart.  Counts beyond 0 .. rows_per_expert are taken as the nearer
+ * of the two.
  * Both enqueue one kernel on stream_ptr, allocate nothing and may be recorded
  * into a graph. */
 int mc_ep_expert_gate_up(uint64_t packed_recv_x_ptr, uint64_t packed_recv_x_scales_ptr,

@@ -52,10 +52,13 @@ __host__ __device__ __forceinline__ float plan_time(int tiles, uint64_t cost, in
     return rounds * ((float)cost * price_reciprocal((float)(tiles > 0 ? tiles : 1)) * steps + kTileCost);
 }
 
-// Few rows (all experts' are one tile each, and at most 32): the weights are read once and are the whole cost.  Where a
-// call reads more of them than the last-level cache is likely to keep until the next, they are read without a place in
-// the caches (8 experts of 44 MB fp8: 58 + 27 us kept, 53 + 24 not); fewer may be there from the call before (9 of
-// 2.2 MB: 10.7 + 7.4 us kept, 12.5 + 8.1 not).
+// Few rows (all experts' are one tile each, and at most 32): the weights are read once and are the whole cost, and they can
+// be read without a place in the caches.  That pays wherever they are not in the last-level cache (256 MiB) already - a
+// product of 50 to 450 MiB after others' weights: 4 to 13 % (8 experts of fp8 7168 x 2048, a row each: 224 + 112 MiB, 56 + 25 us
+// kept, 52 + 23 not; 28 MiB the same, 45) - and costs where they are: up to 250 MiB read again at once 38 us kept and 52
+// not, 12 + 7 for 20 MB (11 + 7), beyond what the cache holds 66 and 59.  Weights that are read again before 256 MiB of
+// others are those of a program of few, small layers: a product of 64 MiB or more is a layer or two of it at most.  (Tiles
+// of 128 weight rows have no such form: they are chosen for products of too few tiles to be bound by the reads.)
 constexpr int64_t kStreamed = 64 << 20;
 __host__ __device__ __forceinline__ bool streamed(int tiles, int experts, int across, int weight_rows, int row_bytes) {
     return tiles == experts && (int64_t)tiles * across * weight_rows * row_bytes >= kStreamed;

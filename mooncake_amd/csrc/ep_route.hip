@@ -14,9 +14,9 @@
 // What bounds it: a token's logits are read once and stay in registers; the arithmetic of the scores and of K dependent
 // searches is what costs, so values are compared as integers in the floats' order, a search is one instruction per
 // halving of the wave and scalar instructions besides, and a lane's values are put in order once.  131072 tokens: 256
-// experts, sigmoid, bias, eight groups 79-84 us (1.7 TB/s of logits; some 440 vector instructions a token, a third of them
-// the scores), softmax without groups 65; 128 experts 53, 64 experts 44, 512 experts 104.  4096 tokens of 256 5.2 us
-// and fewer 5.0, which is the host's call (3.0 from a graph).
+// experts, sigmoid, bias, eight groups 80-85 us (1.7 TB/s of logits; 420 vector instructions a token, a third of them the
+// scores, issued at 1.2 a CU cycle, which is all there is), softmax without groups 65; 128 experts 54, 64 experts 44, 512
+// experts 106.  4096 tokens of 256 5.5 us and fewer 5.3, which is the host's call (3.0 from a graph).
 #include "../../include/mooncake_ep_hip.h"
 
 #include <hip/hip_runtime.h>

@@ -50,15 +50,15 @@ def route(logits: torch.Tensor, num_topk: int, score: str = "softmax", bias: Opt
           num_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0,
           token_mask: Optional[torch.Tensor] = None, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
           ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Router logits [T, E] (f32 or bf16, any row stride) -> (topk_idx int64, topk_weights f32), both [T, num_topk]:
+    """Router logits [T, E] (f32 or bf16, rows any E or more elements apart) -> (topk_idx int64, topk_weights f32), both [T, num_topk]:
     what `Buffer.dispatch` and `Buffer.combine` take.
 
     The scores are softmax (over the experts) or sigmoid of the logits, in 32 bits (a sigmoid is zero for logits below
-    -88.72).  Experts are chosen by score + bias
-    (bias f32 [E]) or, without one, by their logits - the same order -, in falling order, the lowest index first among
-    equals.  With num_groups > 1 the experts are that many equal groups of consecutive ones and only those of the best
-    topk_groups groups can be chosen; a group counts as its best expert, with a bias as its best two together.  The
-    weights are the chosen experts' scores without the bias, divided by their sum if `renormalize`, times `scale`.
+    -88.72).  Experts are chosen by score + bias (bias f32 [E]) or, without one, by their logits - the same order -, in
+    falling order, the lowest index first among equals.  With num_groups > 1 the experts are that many equal groups of
+    consecutive ones and only those of the best topk_groups groups can be chosen; a group counts as its best expert, with
+    a bias as its best two together.  The weights are the chosen experts' scores without the bias, divided by their sum if
+    `renormalize`, times `scale`.
 
     token_mask (bool [T]): False leaves a token out.  Logits of -inf or NaN, and choices of -inf or NaN (a bias of -inf
     takes an expert out of service), are never chosen; +inf counts as the largest finite number.  Places that stay empty
@@ -103,7 +103,10 @@ def expert_gate_up(packed_recv_x: Scaled, packed_recv_count: torch.Tensor, w_gat
     column-major per expert).  w_gate_up: [L, 2I, H], Wg's rows first - bf16, or (fp8 values, f32 scales of their 128 x 128
     blocks [L, 2I/128, H/128]) for an fp8 payload.  Returns (or writes to `act`) bf16 [L, R*max, I], or (fp8 values, f32
     scales [L, R*max, I/128]) laid out like the payload, a scale being amax / 448 with amax at least 1e-4.  I is a multiple
-    of 128 in fp8, of 8 in bf16.  `act` may not lie on the payload."""
+    of 128 in fp8, of 8 in bf16.  `act` may not lie on the payload.
+
+    bf16 products are summed in 32 bits.  In fp8 the matrix instruction cuts each of eight consecutive products off 2^-13
+    below the largest of the eight (an error of at most 7 * 2^-13 of that one per eight); all other sums have 32 bits."""
     x, scales = _parts(packed_recv_x)
     w, w_scales = _parts(w_gate_up)
     a, a_scales = (None, None) if act is None else _parts(act)
@@ -157,7 +160,7 @@ def expert_down(act: Scaled, packed_recv_count: torch.Tensor, w_down: Scaled,
 def expert_mlp(packed_recv_x: Scaled, packed_recv_count: torch.Tensor, w_gate_up: Scaled, w_down: Scaled,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`expert_down` of `expert_gate_up`: dispatch's packed rows -> the rows combine reads.  The activations between the
-    two live in memory that torch lends for the call.  A bf16 `out` may be the payload itself."""
+    two live in memory that torch lends for the call, rounded to the payload's type.  A bf16 `out` may be the payload itself."""
     return expert_down(expert_gate_up(packed_recv_x, packed_recv_count, w_gate_up), packed_recv_count, w_down, out)
 
 
